@@ -542,7 +542,8 @@ class GraphDecoder:
         in all; captured on first use): the prompt is padded at its end, which causal attention makes exact -- no real
         position sees the padding, the logits come from position t - 1, and
         the padding's cache rows are overwritten by the decode steps before
-        they are read.
+        they are read.  The decode step is captured after the first prompt that
+        leaves it a position.
         """
         b, t = idx.shape
         if b != self.ids.shape[0]:
@@ -570,7 +571,7 @@ class GraphDecoder:
         self.cache.length = t
         self.length = t
         self.pos.fill_(t)
-        if self.graph is None:
+        if self.graph is None and t < self.max_len:  # (a full cache leaves no position that a step could run at)
             self._capture()
         return logits[:, 0].clone()
 
@@ -612,7 +613,7 @@ class GraphDecoder:
     @torch.inference_mode()
     def decode(self, next_ids: torch.Tensor) -> torch.Tensor:
         """Logits [batch, vocab] of one new token per sequence at the next position."""
-        if self.graph is None:
+        if self.graph is None and self.length < self.max_len:
             raise RuntimeError("GraphDecoder.decode before prefill")
         if self.length >= self.max_len:
             raise ValueError(f"the cache holds {self.max_len} positions")
@@ -628,7 +629,7 @@ class GraphDecoder:
         """Token ids [batch, n]: n greedy steps from ``next_ids``, each replay feeding its argmax to the next."""
         if not self.greedy:
             raise RuntimeError("decode_greedy needs GraphDecoder(..., greedy=True)")
-        if self.graph is None:
+        if self.graph is None and self.length < self.max_len:
             raise RuntimeError("GraphDecoder.decode_greedy before prefill")
         if n < 0 or self.length + n > self.max_len:
             raise ValueError(f"{n} steps from position {self.length} exceed the cache's {self.max_len} positions")
@@ -645,7 +646,7 @@ class GraphDecoder:
         """Token ids [batch, n]: n steps from ``next_ids``, the i-th token drawn by u[:, i] (fp32 [batch, n], in [0, 1))."""
         if self.sampling is None:
             raise RuntimeError("decode_sampled needs GraphDecoder(..., sampling=Sampling(...))")
-        if self.graph is None:
+        if self.graph is None and self.length < self.max_len:
             raise RuntimeError("GraphDecoder.decode_sampled before prefill")
         if u.dim() != 2 or u.shape[0] != self.ids.shape[0]:
             raise ValueError(f"decode_sampled: u must be [{self.ids.shape[0]}, n]")

@@ -159,3 +159,31 @@ def test_refusals(model, dev):
         with pytest.raises(ValueError):
             generate_many(model, prompts)
     assert cache.free_pages == 4
+
+
+@pytest.mark.parametrize("sampling", [True, False])
+@pytest.mark.parametrize("batch,max_len", [(1, 63), (2, 96)])
+def test_a_decoder_whose_first_prompt_fills_the_cache(model, dev, sampling, batch, max_len, monkeypatch):
+    monkeypatch.setattr(model.head, "gemv_max_tokens", 0 if not sampling else model.head.gemv_max_tokens)  # unfused greedy
+    rules = Sampling(temperature=0.9, top_p=0.9)
+    make = lambda: GraphDecoder(model, batch=batch, max_len=max_len, greedy=not sampling,  # noqa: E731
+                                sampling=rules if sampling else None)
+    u = torch.rand(batch, 5, generator=torch.Generator(device=dev).manual_seed(2), device=dev)
+
+    def decode(dec, first, n):
+        return dec.decode_sampled(first, u[:, :n]) if sampling else dec.decode_greedy(first, n)
+
+    full = torch.tensor(_prompts([max_len] * batch), device=dev)
+    dec, fresh = make(), make()
+    logits = dec.prefill(full)
+    with torch.inference_mode():
+        want = model.prefill(full, model.new_cache(batch, max_len), last_only=True)[:, -1]
+    assert ((logits - want).norm() / want.norm()).item() <= 1e-5
+    assert decode(dec, logits.argmax(-1), 0).shape == (batch, 0)
+    with pytest.raises(ValueError, match="positions"):
+        decode(dec, logits.argmax(-1), 1)
+    with pytest.raises(ValueError, match="positions"):
+        dec.decode(logits.argmax(-1))
+    got, ref = (decode(d, d.prefill(full[:, :-5]).argmax(-1), 5) for d in (dec, fresh))
+    assert torch.equal(got, ref)
+    assert torch.equal(decode(dec, dec.prefill(full[:, :-5]).argmax(-1), 5), got)
