@@ -26,6 +26,7 @@ by its fp16 weight cast to fp32 (pollux.py:562-563).
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, fields
 from typing import Any, Callable, Sequence
 
@@ -343,12 +344,18 @@ class PackedPolluxModel(nn.Module):
         return self.logits(x[:, -1:] if last_only else x)
 
     def embed(self, idx: torch.Tensor, pos0: torch.Tensor) -> torch.Tensor:
-        """tok_emb(idx) + pos_emb(positions pos0 .. pos0 + t - 1) (pollux.py:691-693); pos0 a device int64 tensor."""
+        """tok_emb(idx) + pos_emb(positions pos0 .. pos0 + t - 1) (pollux.py:691-693); pos0 a device int64 tensor.
+
+        Ids outside [0, vocab_size) -- sample_rows gives -1 for a row without a
+        distribution, and a captured step feeds it on -- give NaN rows.
+        """
         if not self.tok_emb._materialized:
             return int8_embed(self.tok_emb.weight_int8, self.tok_emb.mu_rows, idx, pos_weight=self.pos_emb.weight,
                               pos0=pos0)
         pos = pos0.reshape(1, 1) + torch.arange(idx.shape[1], device=idx.device).unsqueeze(0)
-        return self.tok_emb(idx) + self.pos_emb(pos)
+        known = idx.clamp(0, self.tok_emb.num_embeddings - 1)  # (a gather from outside the table would fault)
+        x = self.tok_emb(known) + self.pos_emb(pos)
+        return x.masked_fill((known != idx).unsqueeze(-1), math.nan)
 
     def logits(self, x: torch.Tensor) -> torch.Tensor:
         """head(ln_f(x)) (pollux.py:699-700), the norm fused into the INT8 head where that runs."""
@@ -643,7 +650,11 @@ class GraphDecoder:
 
     @torch.inference_mode()
     def decode_sampled(self, next_ids: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
-        """Token ids [batch, n]: n steps from ``next_ids``, the i-th token drawn by u[:, i] (fp32 [batch, n], in [0, 1))."""
+        """Token ids [batch, n]: n steps from ``next_ids``, the i-th token drawn by u[:, i] (fp32 [batch, n], in [0, 1)).
+
+        A sequence whose logits or settings are no distribution draws -1, and
+        from then on -1 until the next prefill; the others are not affected.
+        """
         if self.sampling is None:
             raise RuntimeError("decode_sampled needs GraphDecoder(..., sampling=Sampling(...))")
         if self.graph is None and self.length < self.max_len:

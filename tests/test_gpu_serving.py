@@ -187,3 +187,31 @@ def test_a_decoder_whose_first_prompt_fills_the_cache(model, dev, sampling, batc
     got, ref = (decode(d, d.prefill(full[:, :-5]).argmax(-1), 5) for d in (dec, fresh))
     assert torch.equal(got, ref)
     assert torch.equal(decode(dec, dec.prefill(full[:, :-5]).argmax(-1), 5), got)
+
+
+@pytest.mark.parametrize("batch", [3, 7, 40])
+@pytest.mark.parametrize("materialize", [False, True])
+def test_a_sequence_without_a_distribution_stays_without_one(model, dev, tmp_path, materialize, batch):
+    if materialize:
+        state, _ = pack.pack_state_dict(_dense_state(BIG, 9), dev)
+        plx.write_plx(tmp_path / "dense.plx", pack.pack_config(BIG), state)
+        model = PackedPolluxModel.from_packed_checkpoint(tmp_path / "dense.plx", dev, materialize=True)
+    prompts = torch.tensor(_prompts([9] * batch), device=dev)
+    u = torch.rand(batch, 12, generator=torch.Generator(device=dev).manual_seed(6), device=dev)
+    others = [i for i in range(batch) if i != 1]
+    got = []
+    for middle in (0.7, float("nan")):  # the second sequence's temperature
+        rules = Sampling(temperature=torch.tensor([0.9, middle] + [1.1] * (batch - 2), device=dev), top_p=0.95, repetition_penalty=1.2)
+        dec = GraphDecoder(model, batch=batch, sampling=rules)
+        ids = dec.decode_sampled(dec.prefill(prompts).argmax(-1), u[:, :7])
+        got.append(torch.cat([ids, dec.decode_sampled(ids[:, -1], u[:, 7:])], 1))  # (its last ids fed back by hand)
+    assert (got[0] >= 0).all() and (got[1][1] == -1).all()
+    assert torch.equal(got[0][others], got[1][others])
+    # a prefill starts afresh; then an id that is none, by the caller
+    rules.temperature[1] = 0.7
+    first = dec.prefill(prompts).argmax(-1)
+    assert torch.equal(dec.decode_sampled(first, u[:, :7]), got[0][:, :7])
+    first = dec.prefill(prompts).argmax(-1)
+    first[1] = -1
+    ids = dec.decode_sampled(first, u[:, :7])
+    assert (ids[1] == -1).all() and torch.equal(ids[others], got[0][others, :7])

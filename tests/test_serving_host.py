@@ -69,3 +69,18 @@ def test_a_prompt_that_fills_the_cache(monkeypatch, sampling, max_len, batch):
     assert decode(2).tolist() == [[50, 50] if sampling else [0, 0]] * batch
     with pytest.raises(ValueError, match="positions"):
         decode(1)
+
+
+def test_ids_that_name_no_token_give_nan_rows_of_materialized_weights():
+    # as the packed embedding's kernel does: a row without a distribution draws the id -1, which a replay then embeds
+    model = PackedPolluxModel(CFG)
+    g = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        model.pos_emb.weight.copy_(torch.randn(CFG.seq_len, CFG.n_embd, generator=g))
+    emb = model.tok_emb
+    emb.weight = torch.nn.Parameter(torch.randn(CFG.vocab_size, CFG.n_embd, generator=g).half(), requires_grad=False)
+    emb._materialized = True
+    x = model.embed(torch.tensor([[3, 4], [-1, 239], [0, 240]]), torch.tensor(5)).detach()
+    assert x.isnan().any(-1).tolist() == x.isnan().all(-1).tolist() == [[False, False], [True, False], [False, True]]
+    for at, (t, p) in {(0, 0): (3, 5), (0, 1): (4, 6), (1, 1): (239, 6), (2, 0): (0, 5)}.items():
+        assert torch.equal(x[at], emb.weight[t].float() + model.pos_emb.weight[p])
