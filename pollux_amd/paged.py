@@ -144,7 +144,8 @@ class PagedBatch:
               device=None) -> PagedBatch:
         """The batch of sequences of kv_lens positions, of which the last q_lens are this step's.
 
-        table: int32 [seqs, pages] on the device, or each sequence's list of pages (then ``device`` says where).
+        table: int32 [seqs, pages] on the device, or each sequence's list of pages (then ``device`` says where;
+        positions past the end of a list have no page).
         """
         if len(kv_lens) != len(q_lens) or len(table) != len(kv_lens):
             raise ValueError("PagedBatch.build: one table row, length and number of new tokens per sequence")
@@ -163,7 +164,8 @@ class PagedBatch:
             small = torch.tensor(small, dtype=torch.int32).to(device)
         else:  # the rows, starts, lengths and order in one copy
             width = max((len(t) for t in table), default=0)
-            rows = [p for t in table for p in (*t, *([0] * (width - len(t))))]
+            # (-1 is no page: a list that ends before its sequence does is read as NaN and written nowhere)
+            rows = [p for t in table for p in (*t, *([-1] * (width - len(t))))]
             both = torch.tensor([*rows, *small], dtype=torch.int32).to(device)
             table, small = both[:seqs * width].view(seqs, width), both[seqs * width:]
         return cls(table, small[:seqs + 1], small[seqs + 1:2 * seqs + 1], starts[-1], top, max(kv_lens, default=0),

@@ -508,3 +508,38 @@ def test_another_stream(dev):
             outs.append(paged_attention(q, kv, batch))
     torch.cuda.synchronize()
     assert all(torch.equal(o, ref) for o in outs)
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+@pytest.mark.parametrize("q_lens", [[40, 40], [1, 1], [40, 1]])
+def test_a_page_list_that_ends_before_its_sequence(dev, kv_dtype, q_lens):
+    """Beside a longer list: what lies past it is written nowhere and NaN, and page 0 is whose it is."""
+    heads, page, kv_lens = 3, 16, [40, 40]
+    tables = [[0, 1, 2], [3]]  # 40 positions, 16 positions
+    g = torch.Generator(device=dev).manual_seed(19)
+    kv = PagedKV.allocate(5, heads, page, kv_dtype, dev)
+    for t in (kv.k, kv.v, kv.k_scale, kv.v_scale):
+        if t is not None:
+            t.zero_()
+    keys, values = _fill(g, kv, [tables[0]], [40], dev)
+    before = [t.clone() for t in (kv.k, kv.v)]
+    n = sum(q_lens)
+    batch = PagedBatch.build(tables, kv_lens, q_lens, dev)
+    short = PagedBatch.build([tables[1]], kv_lens[1:], q_lens[1:], dev)  # (alone its list does not hold them)
+    x = torch.randn(n, heads * 24, generator=g, device=dev)
+    second = slice(q_lens[0], n)
+    only = PagedBatch(batch.table[1:].contiguous(), torch.tensor([0, q_lens[1]], dtype=torch.int32, device=dev),
+                      batch.kv_len[1:].clone(), q_lens[1], q_lens[1], 40)
+    with pytest.raises(ValueError, match="does not hold"):
+        paged_write(x[second], x[second], kv, short)
+    paged_write(x[second], x[second], kv, only)
+    for t, old in zip((kv.k, kv.v), before):
+        assert torch.equal(t[[0, 1, 2, 4]], old[[0, 1, 2, 4]])
+    held = 16 if q_lens[1] == 40 else 0  # new tokens that have a page
+    for got, want in zip(paged_read(kv, only), (x[second], x[second])):
+        assert torch.equal(got[:held], _stored(want[:held].reshape(-1, heads, 24), kv_dtype).view(held, heads * 24))
+        assert torch.isnan(got[held:]).all()
+    q = torch.randn(n, heads * 24, generator=g, device=dev)
+    got = paged_attention(q, kv, batch)
+    _check(got[:q_lens[0]], _reference(q[:q_lens[0]], keys, values, [40], q_lens[:1], None), values, "the longer list")
+    assert torch.isfinite(got[second][:held]).all() and torch.isnan(got[second][held:]).all()

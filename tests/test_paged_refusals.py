@@ -117,3 +117,12 @@ def test_python_checks():
         PagedBatch.build([[0]], [3], [-1], "cpu")
     with pytest.raises(ValueError, match="ROCm device"):
         PagedBatch.build([[0]], [3], [1], "cpu")
+
+
+def test_short_page_lists_end_in_no_page(monkeypatch):
+    # (0 is a page, another sequence's)
+    monkeypatch.setattr(_lib, "require_device", lambda t, what: None)
+    batch = PagedBatch.build([[5, 0, 2], [3], []], [40, 40, 0], [1, 1, 0], "cpu")
+    assert batch.table.tolist() == [[5, 0, 2], [3, -1, -1], [-1, -1, -1]]
+    given = torch.tensor([[5, 0], [3, 0]])
+    assert PagedBatch.build(given, [20, 9], [1, 1]).table.tolist() == [[5, 0], [3, 0]]
