@@ -119,6 +119,18 @@ __device__ __forceinline__ bool sequence(const Batch &b, int r, int &row0, int &
          len <= b.max_kv;
 }
 
+// NaN into head h of all the rows that cu_q gives a sequence out of bounds (its new tokens may be more than max_q), as far
+// as they are the batch's: those from `at` on, `step` apart.
+template <class TX>
+__device__ __forceinline__ void nan_rows(TX *out, const Batch &b, int heads, int h, int row0, int n, int64_t at,
+                                         int64_t step) {
+  if (row0 < 0) return;
+  const float nan = __builtin_nanf("");
+  for (int64_t i = at; i < n && row0 + i < b.tokens; i += step)
+#pragma unroll 1
+    for (int d = 0; d < kDim; d += 4) store4(out + ((row0 + i) * heads + h) * kDim + d, nan, nan, nan, nan);
+}
+
 // Page of position j (0 <= j < max_kv) or -1.
 __device__ __forceinline__ int page_of(const Batch &b, const Pages &kv, int r, int j) {
   const int p = b.table[r * b.table_stride + (j >> kv.shift)];
@@ -223,17 +235,18 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(Pages kv, Batch b,
   idx /= head_tiles;
   const int qt = idx % q_tiles, r = idx / q_tiles;
   int row0, n, len;
-  if (!sequence(b, r, row0, n, len)) {  // rows that are the batch's at all: NaN
-    if (row0 < 0 || n < 0) return;
-    len = -1;
-    n = min(n, b.max_q);
+  if (!sequence(b, r, row0, n, len)) {
+    const int h = ht * kWrHeads + (threadIdx.x & 15);
+    if (h < kv.heads)
+      nan_rows(is_v ? v_out : k_out, b, kv.heads, h, row0, n, qt * kWrTok + (threadIdx.x >> 4), int64_t{q_tiles} * kWrTok);
+    return;
   }
 #pragma unroll
   for (int u = threadIdx.x; u < kWrTok * kWrHeads * 3; u += kThreads) {  // 8 values each
     const int o = u % 3, i = qt * kWrTok + u / 3 / kWrHeads, h = ht * kWrHeads + u / 3 % kWrHeads;
-    if (i >= n || h >= kv.heads || static_cast<int64_t>(row0) + i >= b.tokens) continue;
+    if (i >= n || h >= kv.heads) continue;
     const int j = len - n + i;
-    const int page = len < 0 ? -1 : j < 0 ? 0 : page_of(b, kv, r, j);
+    const int page = j < 0 ? 0 : page_of(b, kv, r, j);
     float *dst = (is_v ? v_out : k_out) + ((static_cast<int64_t>(row0) + i) * kv.heads + h) * kDim + 8 * o;
     float x[8];
     if (page < 0 || j < 0) {  // no such page; a token before the sequence's first position
@@ -312,10 +325,7 @@ __global__ __launch_bounds__(kThreads) void paged_decode_kernel(const TX *__rest
   if (r < 0) return;
   int row0, n, len;
   if (!sequence(b, r, row0, n, len) || (alone && n > 1)) {  // (not alone: the chunk kernel has all sequences and answers)
-    if (alone && sp == 0 && row0 >= 0 && tid < kDim / 4)
-      for (int i = 0; i < min(n, b.max_q) && static_cast<int64_t>(row0) + i < b.tokens; ++i)
-        store4(out + ((static_cast<int64_t>(row0) + i) * kv.heads + h) * kDim + 4 * tid, __builtin_nanf(""),
-               __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""));
+    if (alone && sp == 0) nan_rows(out, b, kv.heads, h, row0, n, tid, 64 * W);
     return;
   }
   if (n != 1) return;
@@ -678,12 +688,8 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
   if (r < 0) return;
   int row0, n, len;
   if (!sequence(b, r, row0, n, len)) {
-    if (sp == 0 && row0 >= 0 && n >= 1) {
-      for (int i = qt * kQ + tid; i < min(n, (qt + 1) * kQ) && static_cast<int64_t>(row0) + i < b.tokens; i += kThreads)
-        for (int d = 0; d < kDim; d += 4)
-          store4(out + ((static_cast<int64_t>(row0) + i) * kv.heads + h) * kDim + d, __builtin_nanf(""),
-                 __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""));
-    }
+    if (sp == 0)
+      nan_rows(out, b, kv.heads, h, row0, n, int64_t{qt} * kThreads + tid, int64_t{q_tiles} * kThreads);
     return;
   }
   if (qt * kQ >= n || (n == 1 && skip_one)) return;

@@ -7,11 +7,13 @@ scores of a few units; sums of probabilities and values add a few 2^-24.  So 128
 over all (fp32 outputs); fp16 and bf16 outputs add half a step of their type, eps / 2 of the value.
 """
 
+import ctypes
 import math
 
 import pytest
 import torch
 
+from pollux_amd import _lib
 from pollux_amd.model import RMSNorm
 from pollux_amd.paged import PagedBatch, PagedKV, paged_attention, paged_read, paged_write
 
@@ -543,3 +545,47 @@ def test_a_page_list_that_ends_before_its_sequence(dev, kv_dtype, q_lens):
     got = paged_attention(q, kv, batch)
     _check(got[:q_lens[0]], _reference(q[:q_lens[0]], keys, values, [40], q_lens[:1], None), values, "the longer list")
     assert torch.isfinite(got[second][:held]).all() and torch.isnan(got[second][held:]).all()
+
+
+def _read_into(kv, batch, rows):
+    """paged_read into outputs of `rows` rows that hold 5."""
+    k, v = (torch.full((rows, kv.heads * 24), 5.0, device=kv.k.device) for _ in range(2))
+    st = _lib.lib().plx_paged_read(ctypes.byref(kv._c), ctypes.byref(batch._c), k.data_ptr(), v.data_ptr(),
+                                   _lib.stream_of(kv.k.device))
+    _lib.check(st, "paged_read")
+    return k, v
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+@pytest.mark.parametrize("ordered", [True, False])
+@pytest.mark.parametrize("kv_len,bounds,new", [
+    (70, [1, 1, 1], [1, 2, 0]), (70, [1, 1, 1], [0, 2, 1]), (5000, [1, 1, 1], [1, 2, 0]),  # one token's kernel
+    (70, [40, 40, 3], [3, 79, 1]), (700, [150, 150, 150], [150, 299, 1]), (5000, [20, 20, 1], [0, 41, 0]),
+    (70, [8, 1, 1], [0, 10, 0])])
+def test_more_new_tokens_than_the_bound(dev, kv_dtype, ordered, kv_len, bounds, new):
+    """All of such a sequence's rows are NaN, also those past max_q and the tiles that it takes; the others are whole."""
+    heads, page = 17, 16
+    g, kv, tables, batch = _setup(dev, [kv_len] * 3, bounds, heads, page, kv_dtype, 23, fill=0.0)
+    keys, values = _fill(g, kv, tables, [kv_len] * 3, dev)
+    if not ordered:
+        batch = PagedBatch(batch.table, batch.cu_q, batch.kv_len, batch.tokens, batch.max_q, batch.max_kv, batch.singles)
+    starts = torch.tensor([0, *new], device=dev).cumsum(0)
+    assert int(starts[-1]) <= batch.tokens and new[1] > batch.max_q
+    batch.cu_q.copy_(starts)
+    a, b, n = starts[1:].tolist()
+    q = torch.randn(batch.tokens, heads * 24, generator=g, device=dev)
+    got = paged_attention(q, kv, batch, out=torch.full_like(q, 5.0))
+    k, v = _read_into(kv, batch, batch.tokens)
+    for t in (got, k, v):
+        assert torch.isnan(t[a:b]).all() and (t[n:] == 5.0).all() and torch.isfinite(t[:a]).all()
+    for at, count, i in ((0, a, 0), (b, n - b, 2)):
+        if not count:
+            continue
+        ref = _reference(q[at:at + count], keys[i:i + 1], values[i:i + 1], [kv_len], [count], None)
+        _check(got[at:at + count], ref, values, f"beside it {kv_dtype} {new}")
+        assert torch.equal(k[at:at + count], keys[i][:, kv_len - count:].transpose(0, 1).reshape(count, -1))
+    before = kv.k.clone(), kv.v.clone()
+    x = torch.randn(batch.tokens, heads * 24, generator=g, device=dev)
+    batch.cu_q.copy_(torch.tensor([0, 0, new[1], new[1]], device=dev))
+    paged_write(x, x, kv, batch)
+    assert torch.equal(kv.k, before[0]) and torch.equal(kv.v, before[1])
