@@ -589,3 +589,24 @@ def test_more_new_tokens_than_the_bound(dev, kv_dtype, ordered, kv_len, bounds, 
     batch.cu_q.copy_(torch.tensor([0, 0, new[1], new[1]], device=dev))
     paged_write(x, x, kv, batch)
     assert torch.equal(kv.k, before[0]) and torch.equal(kv.v, before[1])
+
+
+@pytest.mark.parametrize("kv_dtype", KV)
+def test_tokens_before_the_first_position(dev, kv_dtype):
+    """kv_len below the new tokens: those before position 0 are not written and read as zeros."""
+    kv_lens, q_lens, heads, page = [3, 0, 20], [7, 2, 20], 3, 8
+    g, kv, tables, batch = _setup(dev, kv_lens, q_lens, heads, page, kv_dtype, 29, fill=7.0)
+    before = [t.clone() for t in (kv.k, kv.v, kv.k_scale, kv.v_scale) if t is not None]
+    k, v = (torch.randn(29, heads * 24, generator=g, device=dev) for _ in range(2))
+    paged_write(k, v, kv, batch)
+    for got, x in zip(_read_into(kv, batch, 30), (k, v)):
+        want = _stored(x.view(29, heads, 24), kv_dtype).view(29, -1)
+        want[:4], want[7:9] = 0.0, 0.0
+        assert torch.equal(got[:29], want) and (got[29] == 5.0).all()
+    slots = torch.zeros(kv.k.shape[0], page, dtype=torch.bool, device=dev)
+    for table, n in zip(tables, kv_lens):
+        for j in range(n):
+            slots[table[j // page], j % page] = True
+    for t, old in zip((t for t in (kv.k, kv.v, kv.k_scale, kv.v_scale) if t is not None), before):
+        keep = ~slots[:, None].expand(t.shape[:3])
+        assert torch.equal(t[keep], old[keep])
