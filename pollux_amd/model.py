@@ -712,6 +712,9 @@ def generate_many(model: PackedPolluxModel, prompts: Sequence[Sequence[int]], *,
     if b == 0 or max_new_tokens < 1:
         return out
     rules = sampling if sampling is not None else Sampling(temperature=0.0)
+    for name, value in _rules(rules).items():
+        if isinstance(value, torch.Tensor) and (value.numel() != b or value.device != device):
+            raise ValueError(f"generate_many: {name} must have {b} values on {device}, one per prompt")
     if u is None:
         u = torch.rand(b, max_new_tokens, device=device)
     elif tuple(u.shape) != (b, max_new_tokens) or u.dtype != torch.float32 or u.device != device:

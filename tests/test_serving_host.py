@@ -84,3 +84,13 @@ def test_ids_that_name_no_token_give_nan_rows_of_materialized_weights():
     assert x.isnan().any(-1).tolist() == x.isnan().all(-1).tolist() == [[False, False], [True, False], [False, True]]
     for at, (t, p) in {(0, 0): (3, 5), (0, 1): (4, 6), (1, 1): (239, 6), (2, 0): (0, 5)}.items():
         assert torch.equal(x[at], emb.weight[t].float() + model.pos_emb.weight[p])
+
+
+def test_settings_of_another_number_of_sequences():
+    # (each step selects the settings of the sequences that draw, by index, on the device)
+    model = PackedPolluxModel(CFG)
+    for n in (1, 2, 4):
+        with pytest.raises(ValueError, match="top_k must have 3 values"):
+            pm.generate_many(model, [[1], [2, 3], [4]], sampling=Sampling(temperature=torch.ones(3), top_k=torch.ones(n).long()))
+    with pytest.raises(ValueError, match="temperature must have 3 values"):
+        pm.generate_many(model, [[1], [2, 3], [4]], sampling=Sampling(temperature=torch.ones(3, device="meta")))
