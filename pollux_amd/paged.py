@@ -320,8 +320,13 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _known(self, *seqs: int) -> None:
+        if any(s not in self._tables for s in seqs):
+            raise ValueError("PagedKVCache: no such sequence")
+
     def length(self, seq: int) -> int:
         """Positions that sequence ``seq`` holds."""
+        self._known(seq)
         return self._lengths[seq]
 
     def add(self) -> int:
@@ -332,6 +337,7 @@ class PagedKVCache:
 
     def drop(self, seq: int) -> None:
         """Closes ``seq``; its pages are free for others (work already enqueued on this stream may still read them)."""
+        self._known(seq)
         self._free.extend(reversed(self._tables.pop(seq)))
         del self._lengths[seq]
 
@@ -341,8 +347,7 @@ class PagedKVCache:
             raise ValueError("PagedKVCache.extend: one count per sequence, every sequence once")
         if any(n < 1 for n in counts):
             raise ValueError("PagedKVCache.extend: at least one new token per sequence")
-        if any(s not in self._tables for s in seqs):
-            raise ValueError("PagedKVCache.extend: no such sequence")
+        self._known(*seqs)
         size = self.page_size
         lengths = [self._lengths[s] + n for s, n in zip(seqs, counts)]
         need = [-(-t // size) - len(self._tables[s]) for s, t in zip(seqs, lengths)]

@@ -8,6 +8,7 @@ import torch
 
 from pollux_amd import model as pm
 from pollux_amd.model import GraphDecoder, PackedPolluxModel, PolluxConfig
+from pollux_amd.paged import PagedKVCache
 from pollux_amd.sampling import Sampling
 
 CFG = PolluxConfig(vocab_size=240, tokenizer_vocab_size=230, seq_len=12, n_layers=1, n_heads=2, n_embd=48, d_head=24)
@@ -94,3 +95,15 @@ def test_settings_of_another_number_of_sequences():
             pm.generate_many(model, [[1], [2, 3], [4]], sampling=Sampling(temperature=torch.ones(3), top_k=torch.ones(n).long()))
     with pytest.raises(ValueError, match="temperature must have 3 values"):
         pm.generate_many(model, [[1], [2, 3], [4]], sampling=Sampling(temperature=torch.ones(3, device="meta")))
+
+
+def test_sequences_that_there_are_not():
+    cache = PagedKVCache([SimpleNamespace(k=torch.zeros(4, 2, 8, 24), page_size=8, heads=2)])
+    a, b = cache.add(), cache.add()
+    cache.drop(b)
+    for seq in (b, 99, -1):
+        for call in (lambda: PackedPolluxModel(CFG).extend([[1], [2]], cache, [a, seq]), lambda: cache.length(seq),
+                     lambda: cache.drop(seq), lambda: cache.extend([a, seq], [1, 1])):
+            with pytest.raises(ValueError, match="no such sequence"):
+                call()
+    assert cache.free_pages == 4 and cache.length(a) == 0
