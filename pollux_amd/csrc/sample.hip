@@ -1147,9 +1147,9 @@ int launch_sample_rows(const void *logits, int x_type, int64_t rows, int64_t col
   const SampleArgs a{logits, stride, x_type, static_cast<int>(cols), vec, u, rules, ids, kept, logp};
   const unsigned lds = rules.seen ? static_cast<unsigned>((a.n + 127) / 128 * 16) : 0;
   const auto launch = [&](auto *kernel, unsigned blocks, int threads, size_t fixed) {  // fixed: the kernel's own LDS
-    if (fixed + lds > 65536) {
+    if (fixed + lds > 65536) {  // (the longest row's for any: a call of another thread, of other rows, sets no other value)
       const int st = check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize, kSmMost / 8),
                                "sample_rows: LDS");
       if (st != PLX_OK) return st;
     }
