@@ -497,8 +497,11 @@ int plx_paged_read(const plx_paged_kv *kv, const plx_paged_batch *batch, float *
  * to the token's own (pollux.py:613-626; n: the RMS norm with norm_w, or
  * nothing).  q, out [tokens, heads * 24] of x_type, q's rows `stride` elements
  * apart (0: contiguous), out contiguous and apart from q; both 16-byte aligned.
- * A token before position 0 sees nothing: zeros.  Products and sums in fp32 or better
- * (fp16 parts of 22 bits and more on MFMA), one rounding to x_type.
+ * A token before position 0 sees nothing: zeros.  Products and sums are fp32,
+ * with one rounding to x_type.  Where a sequence brings several tokens each row of 24 of q,
+ * K and V enters its products to 22 bits of its own largest value (two fp16
+ * parts; fp16 rows as they are), whatever other rows hold, and a softmax weight
+ * to 22 bits, or 2^-35 of the largest.
  * workspace: 16-byte aligned, nothing needs clearing; calls that may run at
  * the same time need one each.  The size depends on the shapes and host
  * bounds alone. */

@@ -545,8 +545,10 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(Batch b, int he
 //   Probabilities are 2^(s c - M), one FMA each: M, a scaled maximum less 10, is a rounded number, but the same one
 // for every key, and sums are rescaled by differences of it.  Beside an M of 2^22 and more (a rounding of it would be
 // as large as an exponent) the maximum is taken off before the scale.
-//   A tile with a key or value that is not finite would reach queries that do not see it (0 * inf): such a tile
-// is taken key by key on the VALU.
+//   A tile with a key or value that is not finite would reach queries that do not see it (0 * inf), and so would one far
+// larger than the others, whose parts it would leave without bits: such a tile, or a wave's keys of it, is taken key
+// by key on the VALU.  (The look at each row's largest: 16 INT8 prompts 103.0 -> 104.4 us, a mixed step
+// over fp32 pages 95.1 -> 96.7.)
 //   Bound by VALU issue, not by the matrix products: an exponent, its FMA, its share of the maximum and its two parts are
 // 5 instructions a score; with staging 7.5 (0.5 cycles of a SIMD) for keys of one part, and 13 (0.8) for two, against 0.22
 // and 0.34 cycles of MFMA.  2,045 queries behind 14,339 fp16 keys, 80 heads: 847 us (2.5 billion scores, 74% of the cycles
@@ -609,6 +611,10 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 constexpr float kLift = 10.f, kRise = 5.f;
 
 constexpr uint32_t kInfBits = 0x7F800000u;
+// Of two parts below 2^15 the lower has steps of 2^-24: a row's values keep 22 bits of its largest down to 2^-kDeep of
+// what the parts are scaled by.  The sums of values are held in a unit up to kKeep above the tile's own, and kFall at most
+// below the largest tile's: 2^30 keys of 2^15 times values of 2^15 stay in fp32.
+constexpr int kDeep = 16, kKeep = 3, kFall = 60;
 constexpr int kVRow = 72;  // halves between dims of V^T in LDS (64 keys; 16 rows of a read in distinct banks)
 
 // The state of 32 queries of a wave: lane l holds query l % 32 and, of its sums, the dims with bit 2 equal to l / 32.
@@ -678,6 +684,8 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
   __shared__ __align__(16) uint16_t vt[WK * KP * 25 * kVRow];
   __shared__ __align__(16) uint16_t qs[(kQ + 1) * kQRow];  // the last row: zeros
   __shared__ uint32_t red[2][kThreads / 64];
+  constexpr int kOcts = sizeof(TKV) == 1 ? 1 : 3;         // units that say how large a row is (INT8: each has its scale)
+  __shared__ uint16_t rows[KP == 2 ? kOcts * kTile : 1];  // exponents of a unit's largest: a key's | a value's << 8
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wq = wave % WQ, wk = wave / WQ;
@@ -779,7 +787,7 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
     }
   };
 
-  int ev = -98;  // KP == 2: the sums of values are in units of 2^(ev - 14)
+  int ev = -98, ev_top = -98;  // KP == 2: the sums of values are in units of 2^(ev - 14); the largest ev so far
   if (begin < end) {
     pages(begin);
     load(begin);
@@ -790,13 +798,18 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
 #pragma unroll
     for (int x = 0; x < UN; ++x) {
       const int u = tid + kThreads * x;
-      if (u >= kUnits || base + u % kTile >= end) continue;
-      mk = max(mk, bad[x] ? kInfBits : largest(kraw[x], kscale[x]));
-      mv = max(mv, largest(vraw[x], vscale[x]));
+      if (u >= (sizeof(TKV) == 1 ? kTile : kUnits)) continue;
+      const uint32_t k1 = largest(kraw[x], kscale[x]), v1 = largest(vraw[x], vscale[x]);
+      if constexpr (KP == 2) rows[u] = static_cast<uint16_t>(k1 >> 23 | v1 >> 23 << 8);
+      if (base + u % kTile >= end) continue;
+      mk = max(mk, bad[x] ? kInfBits : k1);
+      mv = max(mv, v1);
     }
     if constexpr (KP == 2) {
-      mk = wave_umax(mk);
-      mv = wave_umax(mv);
+      if (sizeof(TKV) != 1 || 64 * wave < kTile) {  // (INT8: the other waves' units have the same scales)
+        mk = wave_umax(mk);
+        mv = wave_umax(mv);
+      }
     } else {
       mk = __any(max(mk, mv) != 0) ? kInfBits : 0u;
     }
@@ -845,14 +858,31 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
         lfk = part_scale(mk, sizeof(TKV) == 1 ? 7 : 0);
       }
       const int e = 14 - part_scale(mv, sizeof(TKV) == 1 ? 7 : 0);
-      if (e > ev) {
-        const float f = pow2(max(ev - e, -126));
+      if (e > ev || (e < ev - kKeep && mv != 0)) {
+        ev_top = max(ev_top, e);
+        const int to = max(e, ev_top - kFall);
+        const float f = pow2(max(ev - to, -126)), f2 = pow2(min(ev - to + 126, 0));
 #pragma unroll
         for (int i = 0; i < QG; ++i)
 #pragma unroll
-          for (int d = 0; d < 12; ++d) g[i].o[d] *= f;
-        ev = e;
+          for (int d = 0; d < 12; ++d) g[i].o[d] = g[i].o[d] * f * f2;
+        ev = to;
       }
+    }
+    // whether this wave's keys are taken as parts: no row, but one of zeros, lies kDeep below what its parts are scaled by
+    bool parts = finite;
+    if constexpr (KP == 2) {
+      const uint16_t *at = &rows[64 * wk + lane];
+      int k1 = 0, v1 = 0;
+#pragma unroll
+      for (int x = 0; x < kOcts; ++x) {
+        const int y = at[x * kTile];
+        k1 = max(k1, y & 0xFF);
+        v1 = max(v1, y >> 8);
+      }
+      constexpr int kUp = sizeof(TKV) == 1 ? 6 : 0;  // (the largest is 127 scales)
+      const int k_least = 127 - kUp + 14 - lfk - kDeep, v_least = 127 - kUp + ev - kDeep;
+      if (__any(((k1 != 0) & (k1 < k_least)) | ((v1 != 0) & (v1 < v_least)))) parts = false;
     }
     if (finite) {
 #pragma unroll
@@ -901,7 +931,7 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
       const int low = p0 + first(i), top = p0 + min(first(i) + 32, n) - 1;  // the group's positions
       const int pos = low + col;  // (past the last query: masks nothing that is stored)
       if (first(i) >= n || wbase > top) continue;
-      if (finite) {
+      if (parts) {
         const float kfac = pow2(-lfk - 14);
         // the B operands: octets of the query's parts along the contraction, lanes below 32 | from there
         constexpr int kB = KP == 2 ? 5 : 3;

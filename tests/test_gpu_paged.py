@@ -610,3 +610,45 @@ def test_tokens_before_the_first_position(dev, kv_dtype):
     for t, old in zip((t for t in (kv.k, kv.v, kv.k_scale, kv.v_scale) if t is not None), before):
         keep = ~slots[:, None].expand(t.shape[:3])
         assert torch.equal(t[keep], old[keep])
+
+
+@pytest.mark.parametrize("size", [2.0 ** 18, 1e12, 1e30])
+@pytest.mark.parametrize("which", ["key", "value"])
+@pytest.mark.parametrize("kv_dtype", [torch.int8, torch.float32])
+@pytest.mark.parametrize("kv_len,q_len", [(20, 20), (60, 60), (120, 120), (300, 300), (3000, 40), (2500, 200)])
+def test_a_large_row_reaches_no_earlier_token(dev, kv_dtype, kv_len, q_len, which, size):
+    """A key or value far above the others, finite: the tokens before it keep the bar, relative to what they see."""
+    heads, row = 2, kv_len - 6
+    g, kv, tables, batch = _setup(dev, [kv_len], [q_len], heads, 16, kv_dtype, 71)
+    keys, values = _fill(g, kv, tables, [kv_len], dev)
+    q = torch.randn(q_len, heads * 24, generator=g, device=dev)
+    ref = _reference(q, keys, values, [kv_len], [q_len], None)
+    full = PagedBatch.build(tables, [kv_len], [kv_len], dev)
+    k, v = paged_read(kv, full)
+    (k if which == "key" else v)[row] *= size
+    paged_write(k, v, kv, full)
+    before = q_len - 6
+    _check(paged_attention(q, kv, batch)[:before], ref[:before], [x[:, :row] for x in values], f"{which} {size:.0e}")
+
+
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e30])
+@pytest.mark.parametrize("kv_dtype", [torch.int8, torch.float32])
+@pytest.mark.parametrize("kv_len,q_len", [(90, 1), (90, 20), (90, 60), (200, 120), (400, 300), (3000, 40), (2500, 200)])
+def test_a_large_row_of_no_weight(dev, kv_dtype, kv_len, q_len, size):
+    """A key that every query's score is below -10^5 for, its value large: it adds e^-100000 of that, which is nothing,
+    and the others' keys and values, in its tile and in later ones, keep the bar by themselves."""
+    heads, row = 2, 17
+    g, kv, tables, batch = _setup(dev, [kv_len], [q_len], heads, 16, kv_dtype, 73)
+    _fill(g, kv, tables, [kv_len], dev)
+    full = PagedBatch.build(tables, [kv_len], [kv_len], dev)
+    k, v = paged_read(kv, full)
+    k[row], v[row] = -min(size, 1e20), size
+    paged_write(k, v, kv, full)
+    keys, values = (x.view(kv_len, heads, 24).transpose(0, 1) for x in paged_read(kv, full))
+    q = torch.randn(q_len, heads * 24, generator=g, device=dev).abs() + 0.1
+    got = paged_attention(q, kv, batch)
+    ref = _reference(q, [keys], [values], [kv_len], [q_len], None)
+    first = max(0, row + 1 - (kv_len - q_len))
+    others = values.clone()
+    others[:, row] = 0.0
+    _check(got[first:], ref[first:], [others], f"no weight {size:.0e}")
