@@ -1085,19 +1085,20 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
       w.m = mn;
     }
   }
-  const float unit = KP == 2 ? pow2(max(ev - 14, -126)) : 1.f;
+  const float unit = KP == 2 ? pow2(ev - 14) : 1.f;
 #pragma unroll
   for (int i = 0; i < QG; ++i) {
     if (first(i) + col >= n) continue;
     Queries &w = g[i];
     const int64_t row = (static_cast<int64_t>(row0) + first(i) + col) * kv.heads + h;
     const bool sees = p0 + first(i) + col >= 0;
-    if (part) {
+    if (part) {  // (without the lift, which would take sums of values of 10^33 out of fp32)
       float *p = part + (row * splits + sp) * kPart;
+      const float f = pow2(KP == 2 ? ev - 14 - static_cast<int>(kLift) : -static_cast<int>(kLift));
 #pragma unroll
       for (int x = 0; x < 3; ++x)
-        store4(p + 8 * x + 4 * hh, w.o[4 * x] * unit, w.o[4 * x + 1] * unit, w.o[4 * x + 2] * unit, w.o[4 * x + 3] * unit);
-      if (hh == 0) store4(p + kDim, w.m, w.o[12], w.cst, 0.f);
+        store4(p + 8 * x + 4 * hh, w.o[4 * x] * f, w.o[4 * x + 1] * f, w.o[4 * x + 2] * f, w.o[4 * x + 3] * f);
+      if (hh == 0) store4(p + kDim, w.m, w.o[12] * pow2(-static_cast<int>(kLift)), w.cst, 0.f);
     } else {
       const float f = 1.f / w.o[12];
 #pragma unroll

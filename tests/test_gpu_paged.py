@@ -652,3 +652,18 @@ def test_a_large_row_of_no_weight(dev, kv_dtype, kv_len, q_len, size):
     others = values.clone()
     others[:, row] = 0.0
     _check(got[first:], ref[first:], [others], f"no weight {size:.0e}")
+
+
+@pytest.mark.parametrize("kv_dtype", [torch.int8, torch.float32])
+@pytest.mark.parametrize("kv_len,q_len", [(5000, 1), (5000, 33), (5000, 60), (2500, 200), (700, 300)])
+def test_values_near_the_largest_fp32_numbers(dev, kv_dtype, kv_len, q_len):
+    """Values up to 1e33 of one sign, whole and in key ranges: their sums of weights up to 1 stay below 3e38."""
+    heads = 2
+    g, kv, tables, batch = _setup(dev, [kv_len], [q_len], heads, 16, kv_dtype, 79)
+    full = PagedBatch.build(tables, [kv_len], [kv_len], dev)
+    k = torch.randn(kv_len, heads * 24, generator=g, device=dev)
+    v = (0.1 + torch.rand(kv_len, heads * 24, generator=g, device=dev)) * 1e33
+    paged_write(k, v, kv, full)
+    keys, values = (x.view(kv_len, heads, 24).transpose(0, 1) for x in paged_read(kv, full))
+    q = torch.randn(q_len, heads * 24, generator=g, device=dev)
+    _check(paged_attention(q, kv, batch), _reference(q, [keys], [values], [kv_len], [q_len], None), [values], "1e33")
