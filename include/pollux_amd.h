@@ -408,7 +408,8 @@ int plx_argmax_rows(const float *x, int64_t rows, int64_t cols, int64_t *out, vo
  * always the first); min_p leaves those of w >= min(min_p, 1).
  * ids[row] = the first index at which the summed w of what is left passes u
  * times all of it.  temperature 0: the largest z, the lowest index of equal
- * ones.  +inf logits share the draw.  logp[row] (or null): ln of that token's
+ * ones.  +inf logits share the draw; logits of -inf are never among what is
+ * left.  logp[row] (or null): ln of that token's
  * share; kept[row] (or null): how many tokens were left.  A row with a NaN, with
  * no logit above -inf, or with settings that are none (a NaN, a negative
  * temperature, a penalty not above 0) gets the id -1, logp NaN, kept 0.
@@ -462,9 +463,11 @@ typedef struct plx_paged_kv {
  * which attention begins with them (the longest first keeps the card busy to
  * the end); where max_q > 1 its last `singles` must bring one token at most
  * (one of them that brings more gets NaN), and only they take the one-token
- * kernel.  A permutation: a sequence that it does not name gets no output.  A sequence that leaves its bounds, or a page outside the
- * cache: nothing is written to the cache for those tokens, and outputs that
- * depend on it are NaN.  A page that two sequences name (a shared prefix) may
+ * kernel.  A permutation: a sequence that it does not name gets no output.
+ * A sequence that leaves its bounds, or a page outside the cache: nothing is
+ * written to the cache for those tokens, and outputs that depend on it are NaN,
+ * in every row below `tokens` that cu_q gives the sequence.  With seqs or max_q 0
+ * a call does nothing.  A page that two sequences name (a shared prefix) may
  * be read by both; tokens written must have slots of their own.  At most 2^30
  * tokens and positions, 2^24 - 1 sequences, 2^31 - 1 sequences times heads; a
  * call of more than 2^24 blocks is refused as well. */

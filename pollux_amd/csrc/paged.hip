@@ -302,8 +302,10 @@ __device__ __forceinline__ int join_lanes(float (&a)[D], int lane, int first) {
 // 64 / sizeof(TKV) keys, kDecRounds of them at once: one maximum and one rescaling for all), and the lanes' states
 // are joined at the end: their 24 / sizeof(TKV) sums are halved between lane pairs until 3 are left, which takes a
 // quarter of the exchanges of a reduction of all.  W: waves per item; with 1 a block has four items of its own and no
-// barrier, which is faster where items are many and short: the 64 sequences above 40.4 us by four waves, 36.5 by one; but
-// fp32 rows of the same lengths, four times the loads per wave, 36 by four and 47 by one.
+// barrier, which is faster where items are many and short.  64 sequences of up to n positions, 80 heads, us by one wave and
+// by four: INT8 n = 256 14.4 and 35.2, 1,024 30.9 and 44.2, 2,048 59.6 and 67.8, 4,096 109.5 and 113.0; fp16 256 16.0 and
+// 25.0, 1,024 50.4 and 52.0, 2,048 94.2 and 94.0, 4,096 182 and 177; fp32 256 23.8 and 28.7, 512 50.2 and 50.7, 1,024 94.8
+// and 93.4, 2,048 183 and 176.  (One wave from n * sizeof(TKV) of 1,024 down: up to 2,048 it would lose nowhere either.)
 constexpr int kDecRounds = 4;
 template <class TX, class TKV, int W>
 __global__ __launch_bounds__(kThreads) void paged_decode_kernel(const TX *__restrict__ q, int64_t stride,
@@ -551,8 +553,8 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(Batch b, int he
 // over fp32 pages 95.1 -> 96.7.)
 //   Bound by VALU issue, not by the matrix products: an exponent, its FMA, its share of the maximum and its two parts are
 // 5 instructions a score; with staging 7.5 (0.5 cycles of a SIMD) for keys of one part, and 13 (0.8) for two, against 0.22
-// and 0.34 cycles of MFMA.  2,045 queries behind 14,339 fp16 keys, 80 heads: 847 us (2.5 billion scores, 74% of the cycles
-// issue VALU work, 30% MFMA); 16 prompts of up to 1,024 tokens over INT8 pages 104 us (59% and 23%; 38% of the waves' time
+// and 0.34 cycles of MFMA.  2,045 queries behind 14,339 fp16 keys, 80 heads: 829 us (2.5 billion scores, 73% of the cycles
+// issue VALU work, 30% MFMA); 16 prompts of up to 1,024 tokens over INT8 pages 103 us (58% and 23%; 39% of the waves' time
 // is waits).  Four waves per SIMD in place of three would spill 17 registers: 946 -> 1,050 us profiled.
 //   QG groups of 32 queries per wave share a staged tile: the staging, a fifth of the instructions, is then paid half as
 // often.  WQ: with 64 queries or fewer the other waves take other keys, so that none is idle (both sides measured at the rule).
@@ -1127,7 +1129,7 @@ struct Plan {  // how a call's rows are taken: the one-token kernel, the chunk k
 
 int round_up(int64_t x, int64_t m) { return static_cast<int>((x + m - 1) / m * m); }
 
-// lanes that an item's keys fill, up to which one wave takes it (both sides measured at paged_decode_kernel)
+// lanes that an item's keys fill, up to which one wave takes it (both sides at paged_decode_kernel)
 constexpr int64_t kShortItem = 1024;
 
 Plan plan_of(const plx_paged_kv &kv, const plx_paged_batch &b) {

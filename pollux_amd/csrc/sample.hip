@@ -22,12 +22,13 @@
 //   additions, nor on atomics, so a row's token is the same every time, and in any
 //   batch.  The exponential is taken in fp64 to 2^-44, as the error of a 32-bit
 //   one moves borders between tokens by 2^-20 and more: a table of 2^(i / 256) and
-//   a short polynomial (fp64 issues at half rate; a polynomial alone, of degree 9,
-//   took 512 rows of 50,688 tokens 58 us in place of 51).
+//   a short polynomial (a polynomial alone, of degree 9, took 512 rows of 50,688
+//   tokens 58 us in place of 51; an fp64 FMA issues as often as an fp32 one here:
+//   29.5 and 32.7 * 10^12 a second measured).
 //
 //   What bounds it: one row is a chain of four launches (24 us for 50,257 tokens
-//   with every rule, 4 to 6 us each); 512 rows are bound by the exponentials' issue,
-//   31 of 51 us (52 MB of bf16 logits would take 10).  Before the passes had
+//   with every rule, 5 to 8 us each); 512 rows by the pass that takes the exponentials,
+//   32 of 51 us (52 MB of bf16 logits would take 10).  Before the passes had
 //   many blocks, a block per row took 39 us for one row and 80 for the 512.
 
 #include <type_traits>
@@ -89,8 +90,8 @@ __device__ __forceinline__ void fill_table(double *table) {
 }
 
 // 2^44 2^(d rate / 256), d rate / 256 from -80 to 0: the table's entry times e^x, x = f ln 2 / 256 with |f| <= 1/2.
-// e^x - 1 is x and the rest, below 2^-20 and so good to 2^-44 from fp32: that takes 9 fp64 operations (half rate)
-// where a polynomial alone takes 15.
+// e^x - 1 is x and the rest, below 2^-20 and so good to 2^-44 from fp32: that takes 11 fp64 operations, conversions
+// among them, six fewer than a polynomial alone.
 __device__ __forceinline__ double exp2_scaled(const double *table, double d, double rate) {
   const double round = 6755399441055744.0;  // 1.5 * 2^52: its last bits then hold the rounded integer
   const double r = fma(d, rate, round);
@@ -401,7 +402,8 @@ __global__ __launch_bounds__(kSlThreads) void sample_max_kernel(SampleArgs a, Sc
 }
 
 // The histogram (in LDS, then added up in the scratch: integers, so in any order) of counts for top-k or of weights for
-// top-p; without a rule each group's weight.  Bound by the exponentials: 31 us of the 512 rows', 9 fp64 operations each.
+// top-p; without a rule each group's weight.  32 us of the 512 rows': 33 VALU instructions a token, 11 of them fp64, take
+// 59% of the issue cycles; 37% of the waves' time is waits, as a token above -inf is a branch with a table read of its own.
 template <bool WIDE>
 __global__ __launch_bounds__(kSlThreads) void sample_mass_kernel(SampleArgs a, ScratchShape shape) {
   extern __shared__ __align__(16) uint32_t seen[];

@@ -235,6 +235,7 @@ def paged_read(kv: PagedKV, batch: PagedBatch) -> tuple[torch.Tensor, torch.Tens
     """What the slots of the batch's tokens hold: (keys, values), fp32 [tokens, heads * 24] (plx_paged_read).
 
     A batch whose sequences bring all their positions (q_lens = kv_lens) reads them whole.
+    Rows that cu_q gives to no sequence are not written: they hold anything.
     """
     if batch._index != kv._index:
         raise ValueError("paged_read: the batch and the pages must be on one device")

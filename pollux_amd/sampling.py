@@ -53,7 +53,7 @@ def sample_rows(
     """int64 [rows]: a token per row of logits [rows, width] (fp32, fp16 or bf16), drawn by u [rows] (fp32, in [0, 1)).
 
     In this order: the logits of tokens in ``seen`` (int64 [rows, n], of which
-    the first seen_len -- int64 [rows] or one value -- count) are divided by
+    the first seen_len -- an int64 tensor of rows values, or of one -- count) are divided by
     repetition_penalty where positive and multiplied by it elsewhere;
     temperature; top_k > 0 leaves the k largest (of equal ones the lowest
     indices); top_p < 1 the smallest set of the largest whose probability
@@ -66,7 +66,7 @@ def sample_rows(
     A row without a distribution (a NaN, nothing above -inf, settings that are
     none) gets -1.  ``out``: where to put the tokens.  With ``details``:
     (tokens, log-probability of each among what was left fp32, how many were
-    left int64).
+    left int64; logits of -inf never are).
     """
     _lib.require_device(logits, "sample_rows logits")
     if logits.dim() != 2 or logits.dtype not in _X_TYPES:
