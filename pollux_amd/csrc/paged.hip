@@ -548,9 +548,9 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(Batch b, int he
 // for every key, and sums are rescaled by differences of it.  Beside an M of 2^22 and more (a rounding of it would be
 // as large as an exponent) the maximum is taken off before the scale.
 //   A tile with a key or value that is not finite would reach queries that do not see it (0 * inf), and so would one far
-// larger than the others, whose parts it would leave without bits: such a tile, or a wave's keys of it, is taken key
-// by key on the VALU.  (The look at each row's largest: 16 INT8 prompts 103.0 -> 104.4 us, a mixed step
-// over fp32 pages 95.1 -> 96.7.)
+// larger than the others, whose parts it would leave without bits: such a tile's keys, or those that it would, are taken
+// one by one on the VALU.  (The look at each row's largest costs a mixed step over fp32 pages 1%, INT8 prompts nothing
+// measured; one row of 64 a millionth of the others', in every tile, takes the prompts from 103 to 230 us, one row of 1,000 a million times the others' to 810.)
 //   Bound by VALU issue, not by the matrix products: an exponent, its FMA, its share of the maximum and its two parts are
 // 5 instructions a score; with staging 7.5 (0.5 cycles of a SIMD) for keys of one part, and 13 (0.8) for two, against 0.22
 // and 0.34 cycles of MFMA.  2,045 queries behind 14,339 fp16 keys, 80 heads: 829 us (2.5 billion scores, 73% of the cycles
@@ -871,8 +871,8 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
         ev = to;
       }
     }
-    // whether this wave's keys are taken as parts: no row, but one of zeros, lies kDeep below what its parts are scaled by
-    bool parts = finite;
+    // this wave's keys that are not taken as parts: rows, but those of zeros, kDeep below what their parts are scaled by
+    uint64_t single = finite ? 0 : ~uint64_t{0};
     if constexpr (KP == 2) {
       const uint16_t *at = &rows[64 * wk + lane];
       int k1 = 0, v1 = 0;
@@ -884,7 +884,7 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
       }
       constexpr int kUp = sizeof(TKV) == 1 ? 6 : 0;  // (the largest is 127 scales)
       const int k_least = 127 - kUp + 14 - lfk - kDeep, v_least = 127 - kUp + ev - kDeep;
-      if (__any(((k1 != 0) & (k1 < k_least)) | ((v1 != 0) & (v1 < v_least)))) parts = false;
+      single |= __ballot(((k1 != 0) & (k1 < k_least)) | ((v1 != 0) & (v1 < v_least)));
     }
     if (finite) {
 #pragma unroll
@@ -933,7 +933,7 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
       const int low = p0 + first(i), top = p0 + min(first(i) + 32, n) - 1;  // the group's positions
       const int pos = low + col;  // (past the last query: masks nothing that is stored)
       if (first(i) >= n || wbase > top) continue;
-      if (parts) {
+      if (finite) {
         const float kfac = pow2(-lfk - 14);
         // the B operands: octets of the query's parts along the contraction, lanes below 32 | from there
         constexpr int kB = KP == 2 ? 5 : 3;
@@ -976,6 +976,15 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
 #pragma unroll
             for (int x = 0; x < 16; ++x)
               if (wbase + 32 * kb + 8 * (x / 4) + 4 * hh + x % 4 > pos) s[kb][x] = -INFINITY;
+        }
+        if (KP == 2 && single != 0) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const uint32_t bits = static_cast<uint32_t>(single >> (32 * kb)) >> (4 * hh);
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+              if (bits >> (8 * (x / 4) + x % 4) & 1u) s[kb][x] = -INFINITY;
+          }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -1025,12 +1034,15 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
               w.o = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, bh, w.o, 0, 0, 0);
             }
           }
-      } else {
+        if (KP == 1 || single == 0) continue;
+      }
+      {
         // key by key, each to the queries that see it
         const float vf = KP == 2 ? pow2(14 - ev) : 1.f;
         const TX *src = source(i);
 #pragma unroll 1
         for (int j = wbase; j < min(min(wbase + 64, end), top + 1); ++j) {
+          if (KP == 2 && (single >> (j - wbase) & 1) == 0) continue;
           const int pg = page_of(b, kv, r, j);
           const int64_t at = slot_of(kv, max(pg, 0), h, j);
           const TKV *kp = static_cast<const TKV *>(kv.k) + at * kDim, *vp = static_cast<const TKV *>(kv.v) + at * kDim;
@@ -1041,13 +1053,21 @@ __global__ __launch_bounds__(kThreads, WQ == 4 ? (QG == 1 ? 4 : 3) : 2) void pag
           }
           float t = pg < 0 ? __builtin_nanf("") : 0.f;
 #pragma unroll 1
-          for (int d = 0; d < kDim; ++d) {
-            float x;
-            if constexpr (std::is_same_v<TX, float>) x = src[d];
-            else if constexpr (std::is_same_v<TX, bf16_t>) x = bf16_bits_to_float(src[d].bits);
-            else x = __half2float(src[d]);
-            if (norm_w) x = x * w.qf * norm_w[d];
-            t = fmaf(x * pow2(w.lfq - 14), static_cast<float>(kp[d]) * kq, t);
+          for (int o = 0; o < kDim; o += 8) {
+            float x[8], y[8];
+            load8(src + o, x);
+            if constexpr (sizeof(TKV) == 1) {
+              const uint2 c = *reinterpret_cast<const uint2 *>(kp + o);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = byte_of(e < 4 ? c.x : c.y, e & 3);
+            } else {
+              load8(kp + o, y);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              if (norm_w) x[e] = x[e] * w.qf * norm_w[o + e];
+              t = fmaf(x[e] * pow2(w.lfq - 14), y[e] * kq, t);
+            }
           }
           if (j > pos) continue;
           const float mn = fmaxf(w.m, t);

@@ -667,3 +667,33 @@ def test_values_near_the_largest_fp32_numbers(dev, kv_dtype, kv_len, q_len):
     keys, values = (x.view(kv_len, heads, 24).transpose(0, 1) for x in paged_read(kv, full))
     q = torch.randn(q_len, heads * 24, generator=g, device=dev)
     _check(paged_attention(q, kv, batch), _reference(q, [keys], [values], [kv_len], [q_len], None), [values], "1e33")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -17, 1e-9, 1e-25])
+@pytest.mark.parametrize("kv_dtype", [torch.int8, torch.float32])
+@pytest.mark.parametrize("kv_len,q_len", [(90, 1), (20, 20), (90, 60), (200, 120), (400, 300), (3000, 40), (2500, 200)])
+def test_small_rows_among_others(dev, kv_dtype, kv_len, q_len, size):
+    """Every 16th value is small.  Where all the weight is theirs (scores of 58 more) the others add e^-58 = 2^-83 of
+    theirs, so the bar is relative to the small ones down to 2^-60; where the weights are even, to the others."""
+    heads = 2
+    g, kv, tables, batch = _setup(dev, [kv_len], [q_len], heads, 16, kv_dtype, 83)
+    full = PagedBatch.build(tables, [kv_len], [kv_len], dev)
+    small = (torch.arange(kv_len, device=dev) % 16 == 0)[:, None]
+    v = torch.randn(kv_len, heads * 24, generator=g, device=dev)
+    v = torch.where(small, v * size, v)
+    noise = torch.randn(kv_len, heads * 24, generator=g, device=dev)
+    for k, label in ((noise, "even"), (torch.where(small, 6.0, -6.0) + 0.1 * noise, "all of it")):
+        paged_write(k, v, kv, full)
+        keys, values = (x.view(kv_len, heads, 24).transpose(0, 1) for x in paged_read(kv, full))
+        q = torch.ones(q_len, heads * 24, device=dev) if label == "all of it" else \
+            torch.randn(q_len, heads * 24, generator=g, device=dev)
+        ref = _reference(q, [keys], [values], [kv_len], [q_len], None)
+        bar = values[:, small[:, 0]] if label == "all of it" and size >= 2.0 ** -60 else values
+        err = (paged_attention(q, kv, batch).double() - ref).abs().max().item()
+        print(f"[paged] small {size:.0e} {label}: {err:.2e}", flush=True)
+        assert err <= 128 * 2.0 ** -24 * bar.abs().max().item()
+    # keys that are small: their scores are nothing, beside others of a few units
+    paged_write(torch.where(small, noise * size, noise), v, kv, full)
+    keys, values = (x.view(kv_len, heads, 24).transpose(0, 1) for x in paged_read(kv, full))
+    q = torch.randn(q_len, heads * 24, generator=g, device=dev)
+    _check(paged_attention(q, kv, batch), _reference(q, [keys], [values], [kv_len], [q_len], None), [values], "small keys")
