@@ -550,11 +550,12 @@ __global__ __launch_bounds__(kThreads) void paged_combine_kernel(Batch b, int he
 //   A tile with a key or value that is not finite would reach queries that do not see it (0 * inf), and so would one far
 // larger than the others, whose parts it would leave without bits: such a tile's keys, or those that it would, are taken
 // one by one on the VALU.  (The look at each row's largest costs a mixed step over fp32 pages 1%, INT8 prompts nothing
-// measured; one row of 64 a millionth of the others', in every tile, takes the prompts from 103 to 230 us, one row of 1,000 a million times the others' to 810.)
+// measured; one row of 64 a millionth of the others', in every tile, takes the prompts from 103 to 230 us, one row of 1,000
+// a million times the others' to 810.)
 //   Bound by VALU issue, not by the matrix products: an exponent, its FMA, its share of the maximum and its two parts are
-// 5 instructions a score; with staging 7.5 (0.5 cycles of a SIMD) for keys of one part, and 13 (0.8) for two, against 0.22
+// 5 instructions a score; with staging 7.5 (0.5 cycles of a SIMD) for keys of one part, and 12.3 (0.8) for two, against 0.22
 // and 0.34 cycles of MFMA.  2,045 queries behind 14,339 fp16 keys, 80 heads: 829 us (2.5 billion scores, 73% of the cycles
-// issue VALU work, 30% MFMA); 16 prompts of up to 1,024 tokens over INT8 pages 103 us (58% and 23%; 39% of the waves' time
+// issue VALU work, 31% MFMA); 16 prompts of up to 1,024 tokens over INT8 pages 103 us (57% and 23%; 40% of the waves' time
 // is waits).  Four waves per SIMD in place of three would spill 17 registers: 946 -> 1,050 us profiled.
 //   QG groups of 32 queries per wave share a staged tile: the staging, a fifth of the instructions, is then paid half as
 // often.  WQ: with 64 queries or fewer the other waves take other keys, so that none is idle (both sides measured at the rule).
